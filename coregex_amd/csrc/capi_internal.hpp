@@ -150,7 +150,7 @@ struct Scratch {
   uint32_t* pfTickets = nullptr;   // ... [32][64] ticket counters a cache line apart, one block per launch epoch (scan_fields_wave.hip, round 6)
   uint64_t* pfRec = nullptr; uint64_t pfRecRounds = 0;   // ... 128 records of 16 bytes per round, tagged with the same epoch
   uint64_t* pfStats = nullptr;                           // ... per wave: units that waited, polls (CXG_VERBOSE)
-  uint32_t* pairCtr = nullptr; uint32_t pairSeq = 0;     // scan_teddy_pair.hip: two sets of 8 group counters a cache line apart; launch n claims from set n & 1 and zeroes the other
+  uint32_t* pairCtr = nullptr; uint32_t pairSeq = 0;     // scan_teddy_pair.hip: two group counters a cache line apart; launch n claims from counter n & 1 and zeroes the other
   int64_t* offSpans = nullptr; uint64_t offSpansCap = 0;  // offset captures (scanOffsetCaps): the spans in front of the expansion kernel
   int64_t* nullRows = nullptr; uint64_t nullRowsCap = 0;  // nullable programs (scanNullable): rows of the non-empty variant,
   uint64_t* nullCov = nullptr; uint64_t nullCovCap = 0;   // ... inclusive sums of the positions they cover, + one sum per block of 4096 rows

@@ -42,7 +42,7 @@ int scanDeviceOnce(const cxg_program* p, const void* d_hay, uint64_t len, int64_
   uint32_t lastReason = 0;
   cxgdev::ScanArgs a;
   a.pf_status = nullptr; a.pf_ticket = nullptr; a.pf_ncounters = 0;   // (set per launch by the fields programs' branch below)
-  a.pair_ctr = nullptr; a.pair_seq = 0; a.pair_nctr = 0; a.pair_nbig = 0; a.pair_n6 = 0; a.pair_n4 = 0;
+  a.pair_ctr = nullptr; a.pair_seq = 0; a.pair_nbig = 0; a.pair_n6 = 0; a.pair_n4 = 0;
   std::memset(&a.plan, 0, sizeof a.plan); a.plan_shape = 0;
   a.cc_nr = a.cc_neg = a.cc_pairs = 0; std::memset(a.cc_lo, 0, 4); std::memset(a.cc_hi, 0, 4);
   a.u32_rows = t_u32Rows ? 1u : 0u;
@@ -272,17 +272,15 @@ int scanDeviceOnce(const cxg_program* p, const void* d_hay, uint64_t len, int64_
     static int cus = 0;
     if (cus == 0) { int dev = 0, n = 256; if (hipGetDevice(&dev) == hipSuccess) (void)hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev); cus = n > 0 ? n : 256; }
     if (!s.pairCtr) {
-      HIP_TRY(hipMalloc(reinterpret_cast<void**>(&s.pairCtr), 2 * 8 * cxgdev::kPairCtrStride * sizeof(uint32_t)));
-      HIP_TRY(hipMemsetAsync(s.pairCtr, 0, 2 * 8 * cxgdev::kPairCtrStride * sizeof(uint32_t), stream));
+      HIP_TRY(hipMalloc(reinterpret_cast<void**>(&s.pairCtr), 2 * cxgdev::kPairCtrStride * sizeof(uint32_t)));
+      HIP_TRY(hipMemsetAsync(s.pairCtr, 0, 2 * cxgdev::kPairCtrStride * sizeof(uint32_t), stream));
       s.pairSeq = 0;
     }
     a.pair_ctr = s.pairCtr; a.pair_seq = ++s.pairSeq;
-    // ONE counter: strict ticket order.  With several counters (workgroup b asks counter b & 7 first and STEALS from the others once its own is
-    // exhausted) a workgroup can draw a group in front of one it has scanned and not yet resolved — its own look-back then waits for a group it
-    // holds itself (seen as [21, 21]: a watchdog rerun, on short haystacks where the first claims outnumber the groups).  In ticket order every
-    // workgroup's groups ascend and the smallest uncounted group is always being scanned.  Measured: no difference in time (r06_c44_pair_nctr.txt).
-    static const uint32_t pairNctr = getenv("CXG_PAIR_NCTR") ? static_cast<uint32_t>(atoi(getenv("CXG_PAIR_NCTR"))) : 1u;   // (A/B only: 2, 4 or 8 counters)
-    a.pair_nctr = (a.static_groups && (pairNctr == 2u || pairNctr == 4u || pairNctr == 8u)) ? pairNctr : 1u;
+    // ONE counter, strict ticket order (scan_teddy_pair.hip): every workgroup's groups ascend and the smallest uncounted group is always being
+    // scanned.  Spreading the claims over several counters must not come back: a workgroup that takes from another's counter once its own is
+    // exhausted can draw a group in front of one it has scanned and not yet resolved, and its look-back then waits for itself.  It bought
+    // nothing: 0.406-0.410 ms with 2, 4 or 8 counters against 0.409 with one on 1 GiB and 16 literals.
     le = cxgdev::launch_scan_teddy_pair(a, static_cast<uint32_t>(a.ngroups < static_cast<uint64_t>(cus) ? a.ngroups : static_cast<uint64_t>(cus)), stream);
   }
   else if (gen == 9) {                                              // required literal prefix + anchored DFA (kFlagPrefixLiteral)

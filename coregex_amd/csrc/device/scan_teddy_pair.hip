@@ -136,39 +136,25 @@ __global__ __launch_bounds__(kPThreads, 4) void k_scan_teddy_pair(ScanArgs a) {
   PairWaveLds& L = S.wv[wave];
   const uint64_t etag = static_cast<uint64_t>(a.epoch) << kEpochShift;
 
-  // ---- once per workgroup: claim two groups, the literal tables, the pair table
-  // Groups are claimed from pair_nctr counters — ONE in the product (below); with several (A/B builds of the ladder) counter x hands out groups
-  // x, x + nctr, .. and workgroup b asks counter b & (nctr - 1) and, once that is exhausted, the others in turn: that form can deadlock a
-  // workgroup on its own look-back.  (One counter serves ~20 returning atomics per microsecond: a GiB has 2 200 groups.)
-  const uint32_t nctr = a.pair_nctr, cls = blockIdx.x & (nctr - 1u);
+  // ---- once per workgroup: its first two groups, the literal tables, the pair table
+  // Groups are claimed from ONE counter, in strict ticket order: workgroup b begins with groups b and b + G (G workgroups) without asking
+  // anybody — 2 G simultaneous atomics on one address would take the last of them 25 us —, ticket t is group 2 G + t: every workgroup's groups
+  // ascend, and once all G workgroups run the smallest uncounted group is always being scanned by a workgroup that waits for nobody.  (One counter serves ~20 returning atomics per microsecond: a GiB has 2 200 groups.)
   const uint32_t ngroups32 = static_cast<uint32_t>(a.ngroups);
   const uint64_t ngroups = a.ngroups;
-  uint32_t* const ctr = a.pair_ctr + (a.pair_seq & 1u) * (8u * kPairCtrStride);
-  if (blockIdx.x == 0 && tid < 8) a.pair_ctr[((a.pair_seq + 1u) & 1u) * (8u * kPairCtrStride) + static_cast<uint32_t>(tid) * kPairCtrStride] = 0u;   // the next launch's set
-  auto draw = [&]() -> uint32_t { return __hip_atomic_fetch_add(ctr + cls * kPairCtrStride, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
-  // One counter (the product): workgroup b begins with groups b and b + G (G workgroups) without asking anybody — 2 G simultaneous atomics on
-  // one address would take the last of them 25 us —, ticket t is group 2 G + t: every workgroup's groups ascend, the order of the groups is
-  // the order in which they were handed out, and the smallest uncounted group is always being scanned by a workgroup that waits for nobody.
-  const uint32_t G2 = nctr == 1u ? 2u * gridDim.x : 0u;
-  auto claimed = [&](uint32_t t) -> uint32_t {                      // ticket of the own counter -> group; 0xFFFFFFFF: no group left anywhere
-    if (nctr == 1u) return t + G2 < ngroups32 && t + G2 >= G2 ? t + G2 : 0xFFFFFFFFu;
-    uint32_t g = t * nctr + cls;
-    for (uint32_t k = 1; g >= ngroups32 && k < nctr; k++) {
-      const uint32_t x = (cls + k) & (nctr - 1u);
-      g = __hip_atomic_fetch_add(ctr + x * kPairCtrStride, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) * nctr + x;
-    }
-    return g < ngroups32 ? g : 0xFFFFFFFFu;
+  uint32_t* const ctr = a.pair_ctr + (a.pair_seq & 1u) * kPairCtrStride;
+  if (blockIdx.x == 0 && tid == 0) a.pair_ctr[((a.pair_seq + 1u) & 1u) * kPairCtrStride] = 0u;   // the next launch's counter
+  auto draw = [&]() -> uint32_t { return __hip_atomic_fetch_add(ctr, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+  const uint32_t G2 = 2u * gridDim.x;
+  auto claimed = [&](uint32_t t) -> uint32_t {                      // ticket -> group; 0xFFFFFFFF: no group left
+    return t + G2 < ngroups32 && t + G2 >= G2 ? t + G2 : 0xFFFFFFFFu;
   };
-  uint32_t t0 = 0, t1 = 0;
-  if (tid == 0 && nctr != 1u) { t0 = draw(); t1 = draw(); }       // (consumed behind the image's load)
   const BlobHeader* h = reinterpret_cast<const BlobHeader*>(a.blob);
   for (uint32_t i = tid; i < h->aux_len / 4 && i < kPAuxMax / 4; i += kPThreads)
     reinterpret_cast<uint32_t*>(S.aux)[i] = reinterpret_cast<const uint32_t*>(a.blob + h->aux_off)[i];
-  if (tid == 0) {                                                   // (the tickets have had the image's load to come back)
-    uint32_t g0, g1;
-    if (nctr == 1u) { g0 = blockIdx.x < ngroups32 ? blockIdx.x : 0xFFFFFFFFu; g1 = blockIdx.x + gridDim.x < ngroups32 ? blockIdx.x + gridDim.x : 0xFFFFFFFFu; }
-    else { g0 = claimed(t0); g1 = g0 == 0xFFFFFFFFu ? g0 : claimed(t1); }
-    S.gq[0] = g0; S.gq[1] = g1;
+  if (tid == 0) {
+    S.gq[0] = blockIdx.x < ngroups32 ? blockIdx.x : 0xFFFFFFFFu;
+    S.gq[1] = blockIdx.x + gridDim.x < ngroups32 ? blockIdx.x + gridDim.x : 0xFFFFFFFFu;
   }
   __syncthreads();
   // (The first window is asked for HERE, in front of the table build: its latency hides behind it.)
