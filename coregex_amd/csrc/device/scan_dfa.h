@@ -45,6 +45,15 @@ constexpr int kRecCap = 1024;                 // LDS match records per tile befo
 constexpr int32_t kSerialLimit = 128 * 1024;
 constexpr uint32_t kSerialReads = 1u << 20;   // ... and at most this many one-byte reads beyond the staged window per lane and launch (scan_dfa.hip LdsMem::byte).  (Round 5 tried 3 << 17 to end a quadratic program's call sooner; the ownership searches of input without synchronising bytes legitimately read more than that per lane.)
 constexpr uint32_t kErrSerialLimit = 32u;
+// One byte read beyond the staged window, counted in `slow`: false once the lane's budget is spent (`over` raises kErrSerialLimit), the
+// caller then reads 0 instead of memory.  A reader starts with slow = over = 0.
+#if defined(__HIPCC__)
+__host__ __device__
+#endif
+inline bool spend_serial_read(uint32_t& slow, uint32_t& over) {
+  if (++slow > kSerialReads) { over = 1u; return false; }
+  return true;
+}
 constexpr uint32_t kErrLongMatch = 64u;
 struct WalkLimit { int32_t rend; int32_t flag_at; };
 #if defined(__HIPCC__)

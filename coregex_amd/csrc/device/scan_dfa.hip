@@ -47,8 +47,7 @@ struct LdsMem {
     // synchronising bytes (`\D+?xyz|bc` on text without digits: the lazy alternative stays alive, as in the reference) walks
     // matches x stretch bytes — minutes for 80 KB, with the other workgroups spinning in the look-back until their watchdog
     // fires.  Past the budget the call is refused (kErrSerialLimit -> CXG_E_INPUT) and the remaining reads cost nothing.
-    if (++slow > kSerialReads) { over = 1u; return 0u; }
-    return g[r];
+    return spend_serial_read(slow, over) ? g[r] : 0u;
   }
   __device__ __forceinline__ uint32_t dword(int32_t r) const {
     return *reinterpret_cast<const uint32_t*>(lds + lds_pad(r));

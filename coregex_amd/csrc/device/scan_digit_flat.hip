@@ -41,8 +41,7 @@ struct FlatMem {
   __device__ __forceinline__ uint32_t byte(int32_t r) const {
     if (static_cast<uint32_t>(r) < static_cast<uint32_t>(lim)) return lds[lds_pad2(r)];
     over |= static_cast<uint32_t>(r >= flag_at);
-    if (++slow > kSerialReads) { over = 1u; return 0u; }
-    return g[r];
+    return spend_serial_read(slow, over) ? g[r] : 0u;
   }
   __device__ __forceinline__ uint64_t digits(int32_t w) const { return bits[w]; }
   __device__ __forceinline__ int32_t bitmap_limit() const { return lim; }

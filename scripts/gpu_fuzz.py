@@ -60,6 +60,9 @@ if os.environ.get("FUZZ_FEW"):
     hays = [f[rng.integers(0, len(f), size=int(n))] for f in few for n in (70000, 260000)]
     # ... and two long ones: hundreds of groups in the kernel's dense modes, i.e. several windows of the look-back over maps (round 3)
     hays += [few[4][rng.integers(0, 2, size=2 << 20)], np.frombuffer((b"1." * (1 << 20)), dtype=np.uint8)]
+# Not sent to the device: every search of this program runs to the end of a stretch without digits, so most calls on the periodic haystacks spend
+# the whole read budget (a second and more each) before they are refused.  Its refusal is checked on the CPU twin (tests/test_serial_reads_cpu.py).
+LEFT_OUT = {r"\D+?xyzabcx|bcxy|cxyz|xyza[a-c]"}
 ORACLE_ONLY = bool(os.environ.get('FUZZ_ORACLE_ONLY'))
 seen, n_dev, n_sub, bad = set(), 0, 0, 0
 n_refused = 0
@@ -84,6 +87,8 @@ while len(seen) < npat:
     if pat in seen:
         continue
     seen.add(pat)
+    if pat in LEFT_OUT:
+        continue
     if os.environ.get("FUZZ_TRACE"):                      # which pattern is running (a hang or a very slow program shows as the last line)
         print("[%6.1fs] %r" % (time.time() - t0, pat), file=sys.stderr, flush=True)
     try:

@@ -17,6 +17,8 @@ def lib():
         L = C.CDLL(_PATH)
         L.emu_find_all.restype = C.c_int64
         L.emu_find_all.argtypes = [C.c_char_p, C.c_void_p, C.c_uint64, C.c_int, C.c_void_p, C.c_int64, C.c_int]
+        L.emu_find_all_budget.restype = C.c_int64
+        L.emu_find_all_budget.argtypes = [C.c_char_p, C.c_void_p, C.c_uint64, C.c_void_p, C.c_int64, C.POINTER(C.c_uint32)]
         L.emu_find_all_chain.restype = C.c_int64
         L.emu_find_all_chain.argtypes = [C.c_char_p, C.c_void_p, C.c_uint64, C.c_void_p, C.c_int64, C.c_int, C.c_int]
         L.emu_find_all_chain6.restype = C.c_int64
@@ -67,6 +69,18 @@ def find_all(blob: bytes, hay, chunk: int = 64, flat: int = 0) -> np.ndarray:
         if n <= cap:
             return out[:n].reshape(-1, 2).copy()
         cap = int(n)
+
+
+def find_all_budget(blob: bytes, hay):
+    """Table-walking DFA-pair kernel with its serial-walk budget: (rows or the negative error bit, most bytes a lane read beyond its window)."""
+    a = np.frombuffer(bytes(hay), dtype=np.uint8) if not isinstance(hay, np.ndarray) else np.ascontiguousarray(hay)
+    padded = np.concatenate([a, np.zeros(8, dtype=np.uint8)])
+    cap = 2 * a.size + 2                                             # (no empty rows: a row takes a byte)
+    out = np.empty(cap, dtype=np.int64)
+    reads = C.c_uint32()
+    n = lib().emu_find_all_budget(blob, padded.ctypes.data, a.size, out.ctypes.data, cap, C.byref(reads))
+    assert n != -1, "not a DFA-pair program"
+    return (out[:n].reshape(-1, 2).copy() if n >= 0 else int(n)), int(reads.value)
 
 
 def find_all_submatch(span_blob: bytes, cap_blob: bytes, hay, width: int, chunk: int = 64) -> np.ndarray:

@@ -28,12 +28,52 @@ struct HostMem {
   uint32_t dword(int32_t r) const { uint32_t v; std::memcpy(&v, g + r, 4); return v; }
   int32_t wide_limit(int32_t x) const { return x < lim ? x : lim; }
 };
+// k_scan_dfa's reader with its budget (LdsMem): bytes beyond the staged window are counted, the walk is cut by walk_limit
+struct BudgetMem {
+  const uint8_t* g;
+  int32_t lim, flag_at;
+  mutable uint32_t over = 0, slow = 0, touched = 0;   // touched: reads that reached memory beyond the window
+  uint32_t byte(int32_t r) const {
+    if (static_cast<uint32_t>(r) < static_cast<uint32_t>(lim)) return g[r];
+    over |= static_cast<uint32_t>(r >= flag_at);
+    if (!spend_serial_read(slow, over)) return 0u;
+    touched++;
+    return g[r];
+  }
+  uint32_t dword(int32_t r) const { uint32_t v; std::memcpy(&v, g + r, 4); return v; }
+  int32_t wide_limit(int32_t x) const { return x < lim ? x : lim; }
+};
 struct VecSink {
   std::vector<int64_t>* out;
   int64_t origin;
   void emit(int32_t s, int32_t e) { out->push_back(origin + s); out->push_back(origin + e); }
 };
 }  // namespace
+
+// k_scan_dfa on a DFA-pair program: values written, or -kErrSerialLimit where a lane's walk was cut (the host returns CXG_E_INPUT).
+// *max_reads: the largest number of bytes one lane read beyond its staged window.
+extern "C" int64_t emu_find_all_budget(const uint8_t* blob, const uint8_t* hay, uint64_t len, int64_t* out, int64_t cap_vals, uint32_t* max_reads) {
+  const BlobHeader* h = reinterpret_cast<const BlobHeader*>(blob);
+  if (h->magic != kBlobMagic || h->kind != kKindBidir) return -1;
+  std::vector<int64_t> res;
+  uint32_t over = 0;
+  *max_reads = 0;
+  for (uint64_t tile_lo = 0; tile_lo < len; tile_lo += kTile) {
+    const WalkLimit wl = walk_limit(len - tile_lo, kTile + kHalo);
+    VecSink sink{&res, static_cast<int64_t>(tile_lo)};
+    for (int lane = 0; lane < kThreads; lane++) {
+      BudgetMem m{hay + tile_lo, wl.rend < kTile + kHalo ? wl.rend : kTile + kHalo, wl.flag_at};
+      DfaView f{blob + h->fwd_off, 256, h->fwd_start, h->fwd_first_accept};
+      DfaView r{blob + h->rev_off, 256, h->rev_start, h->rev_first_accept};
+      lane_bidir(m, f, r, blob + h->info_off, lane * kChunk, (lane + 1) * kChunk, wl.rend, tile_lo == 0 && lane == 0, sink);
+      over |= m.over;
+      if (m.touched > *max_reads) *max_reads = m.touched;
+    }
+  }
+  if (over) return -static_cast<int64_t>(kErrSerialLimit);
+  for (size_t i = 0; i < res.size() && static_cast<int64_t>(i) < cap_vals; i++) out[i] = res[i];
+  return static_cast<int64_t>(res.size());
+}
 
 extern "C" int64_t emu_find_all(const uint8_t* blob, const uint8_t* hay, uint64_t len, int chunk, int64_t* out,
                                 int64_t cap_vals, int flat) {
