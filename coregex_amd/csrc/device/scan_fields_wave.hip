@@ -835,8 +835,7 @@ __device__ __forceinline__ bool pf_wait_over(const ScanArgs& a, uint64_t t0) { r
 // Round 6 built the kernel with CLAIMED units (tickets; below, -DCXG_PF_TICKETS=1) — a wave that holds unit u then only ever waits for smaller
 // units, which removes the need for a co-resident grid — and measured it against the static assignment (unit = round * W + wave):
 //   * a returning atomic on ONE address is served ~20 times per microsecond; a 6 TB/s scan in 34 KiB units asks ~190 times: 8 counters
-//     cost a pure streaming kernel 25 %, 64 counters a cache line apart 2 % (scripts/microbench/ticket_atomics.hip; scalar s_atomic_add
-//     works on gfx950 and behaves the same);
+//     cost a pure streaming kernel 25 %, 64 counters a cache line apart 2 % (scripts/microbench/ticket_atomics.hip);
 //   * with the counters fast, the ORDERING is what costs: rows can only be written once every smaller unit has been counted, and with one
 //     unit of slack (two parked row lists fill the LDS that six workgroups per CU leave) every unit ends up waiting for the slowest of the
 //     ~6 000 units in flight — 16 GiB: 5.9 ms with a counter per workgroup, 4.8 with the counters asked in rotation, 3.9 with every unit

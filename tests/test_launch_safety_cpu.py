@@ -38,3 +38,12 @@ def test_no_script_or_document_offers_several_group_counters():
     names = [n for n in _tracked(".hip", ".h", ".hpp", ".cc", ".py", ".sh") if n != here] + ["README.md"]
     offers = [n for n in names if re.search(rb"PAIR_NCTR|pair_nctr\b", _read(n))]
     assert offers == []
+
+
+# ---- device code writes through vector stores only: nothing goes through the scalar data cache (its stores, atomics, write-back, discard)
+
+def test_no_source_writes_through_the_scalar_data_cache():
+    names = _tracked(".hip", ".cc", ".cpp", ".h", ".hpp", ".c", ".s", ".S", ".py", ".sh", "Makefile")
+    scalar_write = re.compile(rb"\bs_(?:buffer_|scratch_)?(?:store|atomic)_\w+|\bs_dcache_(?:wb|discard)\w*")
+    assert len(names) > 100
+    assert [(n, m.group().decode()) for n in names for m in [scalar_write.search(_read(n))] if m] == []
