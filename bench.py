@@ -402,10 +402,13 @@ def _check_all_rows(pattern, synth, seed, first_page, npages, out, nmatch, width
 
 def _relaunch_one_rank_per_gpu(n, script, need_gpus=True):
     """`python bench.py --gpus N` without a launcher around it: start N ranks of this very command line under
-    torch.distributed.run (one process per GPU, rendezvous on 127.0.0.1) and become that launcher.  Fails loudly
+    torch.distributed.run (one process per GPU, rendezvous on 127.0.0.1) as a child, and end with its status.  (A child and
+    not an exec: counting the devices may have initialised the GPU, and such a process must not be replaced.)  Fails loudly
     when the node shows fewer than N devices — N ranks never share a GPU.  (`script`, `need_gpus`: tests/bench_stub.py runs
     the same launcher and timing protocol on CPU with a workload that sleeps.)"""
+    import signal
     import socket
+    import subprocess
     if need_gpus:
         import torch
         have = torch.cuda.device_count()
@@ -419,7 +422,21 @@ def _relaunch_one_rank_per_gpu(n, script, need_gpus=True):
     env = dict(os.environ)
     env.setdefault("HSA_ENABLE_IPC_MODE_LEGACY", "0")              # RCCL on this pool: dmabuf IPC only
     env.setdefault("OMP_NUM_THREADS", "1")
-    os.execvpe(cmd[0], cmd, env)
+    child, early = None, []
+
+    def forward(sig, _frame):                                        # a signal to this process alone must not leave the ranks running
+        if child is None:
+            early.append(sig)
+        else:
+            child.send_signal(sig)
+    for sig in (signal.SIGTERM, signal.SIGHUP):
+        signal.signal(sig, forward)
+    signal.signal(signal.SIGINT, lambda sig, frame: None)            # the terminal sends it to the launcher as well
+    child = subprocess.Popen(cmd, env=env)
+    for sig in early:
+        child.send_signal(sig)
+    rc = child.wait()
+    raise SystemExit(rc if rc >= 0 else 128 - rc)
 
 
 def _cpu_baseline(config, cfg, pattern, buf, out, nmatch, nbytes, width, base, synth, seed):
