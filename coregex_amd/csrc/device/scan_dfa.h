@@ -25,6 +25,24 @@ constexpr uint64_t kWaveGroupBytes = static_cast<uint64_t>(kWaveTile) * kWavesPe
 constexpr int kPairWaves = 16;
 constexpr int kPairTilesPerWave = 8;
 constexpr uint32_t kPairCtrStride = 32;       // uint32 between two group counters (128 bytes)
+// How its workgroups come by their groups.  G workgroups, static start: workgroup b begins with groups b and b + G without asking anybody (2 G
+// simultaneous atomics on one address would take the last of them 25 us), ticket t of the one counter is group 2 G + t.  Without it (after a
+// watchdog hit, or with CXG_TICKETS) every group is a ticket.  kPairNoGroup: none left.
+constexpr uint32_t kPairNoGroup = 0xFFFFFFFFu;
+#if defined(__HIPCC__)
+__host__ __device__
+#endif
+inline uint32_t pair_static_group(uint32_t wg, uint32_t k, uint32_t nwg, uint32_t ngroups) {   // k = 0, 1
+  const uint32_t g = wg + k * nwg;
+  return g < ngroups ? g : kPairNoGroup;
+}
+#if defined(__HIPCC__)
+__host__ __device__
+#endif
+inline uint32_t pair_ticket_group(uint32_t ticket, uint32_t nwg, uint32_t ngroups, bool static_start) {
+  const uint32_t first = static_start ? 2u * nwg : 0u, g = first + ticket;
+  return g < ngroups && g >= first ? g : kPairNoGroup;
+}
 constexpr uint64_t kPairGroupBytes = static_cast<uint64_t>(kWaveTile) * kPairWaves * kPairTilesPerWave;
 #ifndef CXG_PAIR_SMALL_TPW
 #define CXG_PAIR_SMALL_TPW 2               // (A/B builds: 4)

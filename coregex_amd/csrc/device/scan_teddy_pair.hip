@@ -28,8 +28,9 @@
 // consecutive wave-tiles (480 KiB), and small ones of 2-tile units for the haystack's last stretch — are CLAIMED through
 // one atomic counter, two claims ahead, the first two groups of a workgroup without an atomic (the ticket is drawn by one lane a group early; this file is compiled with
 // -amdgpu-atomic-optimizer-strategy=None: the optimizer's wave reduction waited for the ticket, and for every window load
-// in flight, on the spot).  A workgroup that holds group g only ever waits for groups < g, which are held by running
-// workgroups: forward progress does not depend on co-residency or on the order of dispatch.  The
+// in flight, on the spot).  A workgroup that holds group g only ever waits for groups < g: those of workgroups that run, and the
+// first two of every workgroup of the grid.  A grid that is not wholly resident (CUs held by a foreign kernel) can therefore run
+// into the spin limit; the call is then launched again with every group a ticket, and that form needs no co-residency.  The
 // tables come with the program image (built on the host: program.cc buildPairImage).  A wave scans one unit per group behind ONE buffer descriptor, in a two-tile loop body:
 // filter(j + 1) runs between the REQUEST of the 16 bytes at each candidate of tile j (global memory; there is no room for an
 // LDS copy of the window) and their comparison.  The rows of a group are ordered with the decoupled look-back of
@@ -137,24 +138,23 @@ __global__ __launch_bounds__(kPThreads, 4) void k_scan_teddy_pair(ScanArgs a) {
   const uint64_t etag = static_cast<uint64_t>(a.epoch) << kEpochShift;
 
   // ---- once per workgroup: its first two groups, the literal tables, the pair table
-  // Groups are claimed from ONE counter, in strict ticket order: workgroup b begins with groups b and b + G (G workgroups) without asking
-  // anybody — 2 G simultaneous atomics on one address would take the last of them 25 us —, ticket t is group 2 G + t: every workgroup's groups
-  // ascend, and once all G workgroups run the smallest uncounted group is always being scanned by a workgroup that waits for nobody.  (One counter serves ~20 returning atomics per microsecond: a GiB has 2 200 groups.)
+  // Groups are claimed from ONE counter, in strict ticket order (scan_dfa.h pair_static_group / pair_ticket_group): every workgroup's groups
+  // ascend, and the smallest uncounted group is held by a workgroup that waits for nobody — by one that RUNS if every group is a ticket; with
+  // the static start that takes a grid that is wholly resident, and one that is not ends at the spin limit and is launched again on tickets
+  // alone.  (One counter serves ~20 returning atomics per microsecond: a GiB has 2 200 groups.)
+  const bool static_start = a.static_groups != 0u;
   const uint32_t ngroups32 = static_cast<uint32_t>(a.ngroups);
   const uint64_t ngroups = a.ngroups;
   uint32_t* const ctr = a.pair_ctr + (a.pair_seq & 1u) * kPairCtrStride;
   if (blockIdx.x == 0 && tid == 0) a.pair_ctr[((a.pair_seq + 1u) & 1u) * kPairCtrStride] = 0u;   // the next launch's counter
   auto draw = [&]() -> uint32_t { return __hip_atomic_fetch_add(ctr, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
-  const uint32_t G2 = 2u * gridDim.x;
-  auto claimed = [&](uint32_t t) -> uint32_t {                      // ticket -> group; 0xFFFFFFFF: no group left
-    return t + G2 < ngroups32 && t + G2 >= G2 ? t + G2 : 0xFFFFFFFFu;
-  };
+  auto claimed = [&](uint32_t t) -> uint32_t { return pair_ticket_group(t, gridDim.x, ngroups32, static_start); };
   const BlobHeader* h = reinterpret_cast<const BlobHeader*>(a.blob);
   for (uint32_t i = tid; i < h->aux_len / 4 && i < kPAuxMax / 4; i += kPThreads)
     reinterpret_cast<uint32_t*>(S.aux)[i] = reinterpret_cast<const uint32_t*>(a.blob + h->aux_off)[i];
   if (tid == 0) {
-    S.gq[0] = blockIdx.x < ngroups32 ? blockIdx.x : 0xFFFFFFFFu;
-    S.gq[1] = blockIdx.x + gridDim.x < ngroups32 ? blockIdx.x + gridDim.x : 0xFFFFFFFFu;
+    if (static_start) { S.gq[0] = pair_static_group(blockIdx.x, 0u, gridDim.x, ngroups32); S.gq[1] = pair_static_group(blockIdx.x, 1u, gridDim.x, ngroups32); }
+    else { S.gq[0] = claimed(draw()); S.gq[1] = claimed(draw()); }
   }
   __syncthreads();
   // (The first window is asked for HERE, in front of the table build: its latency hides behind it.)
@@ -230,7 +230,7 @@ __global__ __launch_bounds__(kPThreads, 4) void k_scan_teddy_pair(ScanArgs a) {
     auto filter = [&](int j, uint32_t cb_, TileCtx& cx) {
       lane = lane0;
       asm volatile("" : "+v"(lane));                                // (scan_chain_wave.hip: no hoisted-and-spilled lane constants)
-      // the loads of the next tile (the unit behind this one may lie anywhere in the haystack — a stolen claim —, also when this tile lies behind its end)
+      // the loads of the next tile (the unit behind this one may lie anywhere in the haystack, also when this tile lies behind its end)
       auto issue_next = [&]() { if (j + 1 < cur.tiles) issue_loads(cur, j + 1); else { nxt = make_unit(next_group); issue_loads(nxt, 0); } };
       const int32_t rend = cur.rem - j * kWaveTile;
       const bool first_tile = j == 0 && cur.pre == 0;               // the haystack's first tile (or a unit behind its end)

@@ -17,6 +17,9 @@ def lib():
         L = C.CDLL(_PATH)
         L.emu_find_all.restype = C.c_int64
         L.emu_find_all.argtypes = [C.c_char_p, C.c_void_p, C.c_uint64, C.c_int, C.c_void_p, C.c_int64, C.c_int]
+        for name in ("emu_pair_static_group", "emu_pair_ticket_group"):
+            getattr(L, name).restype = C.c_uint32
+            getattr(L, name).argtypes = [C.c_uint32] * 3 + ([C.c_int] if name.endswith("ticket_group") else [C.c_uint32])
         L.emu_find_all_budget.restype = C.c_int64
         L.emu_find_all_budget.argtypes = [C.c_char_p, C.c_void_p, C.c_uint64, C.c_void_p, C.c_int64, C.POINTER(C.c_uint32)]
         L.emu_find_all_chain.restype = C.c_int64

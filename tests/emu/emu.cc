@@ -50,6 +50,9 @@ struct VecSink {
 };
 }  // namespace
 
+extern "C" uint32_t emu_pair_static_group(uint32_t wg, uint32_t k, uint32_t nwg, uint32_t ngroups) { return pair_static_group(wg, k, nwg, ngroups); }
+extern "C" uint32_t emu_pair_ticket_group(uint32_t ticket, uint32_t nwg, uint32_t ngroups, int static_start) { return pair_ticket_group(ticket, nwg, ngroups, static_start != 0); }
+
 // k_scan_dfa on a DFA-pair program: values written, or -kErrSerialLimit where a lane's walk was cut (the host returns CXG_E_INPUT).
 // *max_reads: the largest number of bytes one lane read beyond its staged window.
 extern "C" int64_t emu_find_all_budget(const uint8_t* blob, const uint8_t* hay, uint64_t len, int64_t* out, int64_t cap_vals, uint32_t* max_reads) {
