@@ -4,7 +4,7 @@
 //   sleepN  the same in every wave of a full grid (what a stalled persistent grid looks like: every wave asleep)
 //   busy    one wave brackets a grid that keeps every SIMD issuing VALU work
 // and the two counters' advance per microsecond of event time in each.
-// hipcc --offload-arch=gfx950 -O3 scripts/microbench/clocks.hip -o scripts/microbench/clocks && scripts/microbench/clocks
+// hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops scripts/microbench/clocks.hip -o scripts/microbench/clocks && scripts/microbench/clocks
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <stdio.h>
