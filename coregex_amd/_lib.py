@@ -65,9 +65,11 @@ class Nfa(C.Structure):
 
 
 def build(force: bool = False) -> str:
-    """Compile libcoregex_hip.so for gfx950 with hipcc (cross-compiles without a GPU)."""
+    """Compile libcoregex_hip.so for gfx950 with hipcc (cross-compiles without a GPU).  `force`: every object, whatever is built."""
     src = os.path.join(_HERE, "csrc")
-    if force or not os.path.exists(LIB_PATH) or _stale(src):
+    if force:
+        subprocess.check_call(["make", "-s", "-B", "-j8", "-C", src])
+    elif not os.path.exists(LIB_PATH) or _stale(src):
         subprocess.check_call(["make", "-s", "-j8", "-C", src])
     return LIB_PATH
 
