@@ -124,7 +124,7 @@ class DeviceWorkload:
         t = self.timing if timed else None
         kw = {} if self.u32 else {"base": self.base}                # compact rows are relative to the shard
         n = self.scan(self.buf.ptr, self.nbytes, self.out.data_ptr(), self.nmatch + 16, stream=0, timing=t, **kw)   # the library's own stream; events are recorded on it
-        assert n == self.nmatch or os.environ.get("CXG_DEBUG"), (n, self.nmatch)
+        assert n == self.nmatch, (n, self.nmatch)
         if timed:
             self.kernels.add(int(t.kernel))
             self.launches = max(self.launches, int(t.n_launches))
@@ -216,7 +216,7 @@ class DeviceWorkload:
         }
         rank, world = self.rank, self.world
         under_profiler = _under_profiler()
-        if rank == 0 and not args.no_pmc and not under_profiler and not os.environ.get("CXG_DEBUG"):
+        if rank == 0 and not args.no_pmc and not under_profiler:
             # HBM traffic of the dominant kernel, measured NOW: two child runs of this very workload under rocprofv3, one PMC
             # counter each (after the timed region; the parent only waits).  The committed profile is the fallback.  With N > 1
             # ranks (round 6) the children run rank 0's shard alone on rank 0's device (HIP_VISIBLE_DEVICES pinned) while the other
@@ -229,9 +229,9 @@ class DeviceWorkload:
                                                            "correction": "FETCH_SIZE x2 (gfx950 reports half of wide coalesced reads, MI355X_MICROARCH.md HBM); WRITE_SIZE as reported"}
             elif result["roofline"]["traffic"] is not None:
                 result["roofline"]["traffic_source"] = "committed profile of the same workload and kernel (profiles/*_pmc_traffic.json); the live rocprofv3 passes failed"
-        if rank == 0 and world == 1 and not args.no_cpu_baseline and args.pattern is None and not self.u32 and not os.environ.get("CXG_DEBUG"):
+        if rank == 0 and world == 1 and not args.no_cpu_baseline and args.pattern is None and not self.u32:
             result["cpu_baseline"] = _cpu_baseline(args.config, self.cfg, self.pattern, self.buf, self.out, nmatch, nbytes, width, self.base, self.synth, self.seed)
-        if args.check_all_rows and not os.environ.get("CXG_DEBUG"):
+        if args.check_all_rows:
             result.setdefault("cpu_baseline", {})["all_rows_check"] = _check_all_rows(self.pattern, self.synth, self.seed, rank * self.npages, self.npages, self.out, nmatch, width, self.base)
 
 
@@ -328,10 +328,10 @@ def main(argv=None, make_workload=DeviceWorkload, script=None):
         result["config"]["per_rank_achieved_GBps"] = [round(b / (ms * 1e-3) / 1e9, 2) for b, ms in zip(per_rank_alg, per_rank_ms)]
         result["config"]["per_rank_roofline_frac"] = [round(b / (ms * 1e-3) / 1e9 / HBM_PEAK_GBS, 4) for b, ms in zip(per_rank_alg, per_rank_ms)]
     wl.finish(result, k_ms)
-    if make_workload is DeviceWorkload and hasattr(wl, "async_leg") and not args.no_async and not wl.submatch and not wl.u32 and not os.environ.get("CXG_DEBUG"):
+    if make_workload is DeviceWorkload and hasattr(wl, "async_leg") and not args.no_async and not wl.submatch and not wl.u32:
         result["async"] = wl.async_leg(args.steps)
     if (make_workload is DeviceWorkload and world == 1 and args.config == 2 and args.pattern is None and args.total_gib == 0 and args.gib_per_gpu == 1.0
-            and not args.u32_rows and not args.no_north_star and not os.environ.get("CXG_DEBUG") and not _under_profiler()):
+            and not args.u32_rows and not args.no_north_star and not _under_profiler()):
         del wl
         result["north_star"] = _north_star(args)
     if rank == 0:

@@ -71,9 +71,7 @@ int scanDeviceOnce(const cxg_program* p, const void* d_hay, uint64_t len, int64_
   a.total = reinterpret_cast<uint64_t*>(s.ctl + 8);
   a.err = reinterpret_cast<uint32_t*>(s.ctl + 16);
   static const bool profOn = getenv("CXG_PROF") != nullptr;
-  static const uint32_t dbgBits = getenv("CXG_DEBUG") ? static_cast<uint32_t>(atoi(getenv("CXG_DEBUG"))) : 0u;
   a.prof = nullptr;
-  a.dbg = dbgBits;
   a.limit = limit > 0 ? static_cast<uint64_t>(limit) : 0;
   a.stop = reinterpret_cast<uint32_t*>(s.ctl + 24);                   // device word of the control block (zeroed with it; epoch-tagged otherwise)
   a.max_len = (h->flags & cxgdev::kFlagBothRestart) ? cxgdev::kBothRestartSpan : 0u;
@@ -147,7 +145,7 @@ int scanDeviceOnce(const cxg_program* p, const void* d_hay, uint64_t len, int64_
   // the wave kernel was ahead below 320 MiB; now the pair kernel is level or ahead from 1 KiB on — r06_c83_pair_sizes_final.txt: 64 KiB 13.6
   // against 23.0 us, 1 MiB 17.4 / 33.7, 64 MiB 43.5 / 48.0, 1 GiB 294 / 405.  CXG_PAIR_MIN_BYTES moves the border for A/B runs.)
   static const uint64_t pairMinBytes = getenv("CXG_PAIR_MIN_BYTES") ? strtoull(getenv("CXG_PAIR_MIN_BYTES"), nullptr, 10) : 0ull;
-  if (gen == 7 && pairOk && reinterpret_cast<const cxgdev::TeddyAux*>(p->blob.data() + h->aux_off)->pair_off != 0u && len >= pairMinBytes && limit <= 0 && !denseChain && !profOn && dbgBits == 0 && p->noPair[submatch ? 1 : 0].load(std::memory_order_relaxed) == 0) gen = 12;
+  if (gen == 7 && pairOk && reinterpret_cast<const cxgdev::TeddyAux*>(p->blob.data() + h->aux_off)->pair_off != 0u && len >= pairMinBytes && limit <= 0 && !denseChain && !profOn && p->noPair[submatch ? 1 : 0].load(std::memory_order_relaxed) == 0) gen = 12;
   uint8_t ladder[sizeof(cxg_timing{}.ladder)] = {0};               // kernel id of every span launch of this call, in order
   uint32_t nladder = 0;
   // One iteration = one span launch (+ its capture pass).  What comes next is decided at the bottom from the kernel's error word:
@@ -161,7 +159,7 @@ int scanDeviceOnce(const cxg_program* p, const void* d_hay, uint64_t len, int64_
   std::memset(a.caps, 0, sizeof a.caps);
   a.static_groups = (gen >= 6 && !staticDenied) ? 1u : 0u;
   OrderGate orderGate(ps, stream);                                 // this iteration's launch section: behind whatever any thread enqueued on the device before (closed once everything is enqueued)
-  Scratch::AsyncSlot* const as = (t_asyncSlot && relaunches == 0 && !submatch && !profOn && !dbgBits && a.max_len == 0) ? t_asyncSlot : nullptr;
+  Scratch::AsyncSlot* const as = (t_asyncSlot && relaunches == 0 && !submatch && !profOn && a.max_len == 0) ? t_asyncSlot : nullptr;
   if (gen == 11 && !a.static_groups) { gen = 10; fsmTried = true; }   // the delimiter kernel has no ticket mode
   a.ngroups = a.ntiles;
   if (gen == 8 || gen == 11) a.ngroups = (len + cxgdev::kCcGroupBytes - 1) / cxgdev::kCcGroupBytes;
@@ -244,7 +242,7 @@ int scanDeviceOnce(const cxg_program* p, const void* d_hay, uint64_t len, int64_
   if (gen == 10) {
     static const bool deepOnly = getenv("CXG_FSM_DEEP") != nullptr;   // A/B: the general event-list instantiation for every machine
     const cxgdev::FsmHeader* fh = reinterpret_cast<const cxgdev::FsmHeader*>(fsmImg.data());
-    fsmDirectRan = fsmDirect && !deepOnly && fh->depth <= 1 && a.prof == nullptr && a.dbg == 0;
+    fsmDirectRan = fsmDirect && !deepOnly && fh->depth <= 1 && a.prof == nullptr;
     fsmDirectTables = fsmDirectRan && fsmDirectOk && fh->direct_off != 0u && fh->nk == 1;
     le = cxgdev::launch_scan_fsm(a, fh->lds_bytes, fh->depth <= 1 && !deepOnly, fh->end_col != 0u ? 2 : (fh->nk > 1 ? 1 : 0), stream, fsmDirectTables ? fh->direct_bytes : 0u, fsmDirectRan, fsmMode);
   }
@@ -330,7 +328,7 @@ int scanDeviceOnce(const cxg_program* p, const void* d_hay, uint64_t len, int64_
     // (TRIO mode: built and measured in round 5 — config 5 0.438 ms against 0.395 on the grouped kernel, `(\d+)\.(\d+)\.(\d+)\.(\d+)` 0.57
     // against 0.44: that mathematics is VALU- and LDS-bound and the persistent instantiation holds half the waves — so off unless asked for)
     static const bool trioPers = getenv("CXG_TRIO_PERS") != nullptr;
-    bool persWanted = (fieldsKernel || litKernel || (trioKernel && trioPers)) && persOk && a.static_groups && a.limit == 0 && a.prof == nullptr && a.dbg == 0 && !persDenied;
+    bool persWanted = (fieldsKernel || litKernel || (trioKernel && trioPers)) && persOk && a.static_groups && a.limit == 0 && a.prof == nullptr && !persDenied;
     if (persWanted && !ps.persistent.allowed()) { ps.persistent.consume(); persDenied = true; persWanted = false; }
     if (persWanted) {
       const uint64_t nwt = (len + cxgdev::kWaveTile - 1) / cxgdev::kWaveTile;
@@ -364,7 +362,7 @@ int scanDeviceOnce(const cxg_program* p, const void* d_hay, uint64_t len, int64_
     }
     if (a.pf_status == nullptr) litKernel = false;                  // no persistent launch for this call: the chain kernel
     static const bool countSumOk = getenv("CXG_NO_COUNT_SUM") == nullptr;
-    a.count_sum = ((fieldsKernel || litKernel || (trioKernel && a.pf_status != nullptr)) && countSumOk && a.out == nullptr && a.max_len == 0 && a.limit == 0 && a.prof == nullptr && !a.dbg) ? 1u : 0u;
+    a.count_sum = ((fieldsKernel || litKernel || (trioKernel && a.pf_status != nullptr)) && countSumOk && a.out == nullptr && a.max_len == 0 && a.limit == 0 && a.prof == nullptr) ? 1u : 0u;
     if (a.u32_rows && a.out != nullptr && !((fieldsKernel || litKernel) && a.pf_status != nullptr)) {
       // the persistent kernel has the compact epilogue; when THIS call cannot have it (a rerun, the mode demoted for a while, FindAll's n) the
       // caller uses cxg_find_all_device for the call (CXG_E_INPUT), the program itself stays served
@@ -595,7 +593,6 @@ int scanDeviceOnce(const cxg_program* p, const void* d_hay, uint64_t len, int64_
     return kRcLongMatch;
   }
   if (err) return fail(CXG_E_INTERNAL, "device-side watchdog/overflow flag " + std::to_string(err));
-  if (dbgBits) { if (n_out) *n_out = total; return CXG_OK; }
   uint64_t n = total;
   if (limit > 0 && n > static_cast<uint64_t>(limit)) n = static_cast<uint64_t>(limit);
   if (n_out) *n_out = n;

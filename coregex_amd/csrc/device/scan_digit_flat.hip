@@ -166,7 +166,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_digit_flat(ScanArgs a) {
   const bool at_origin = (tile_lo == 0 && tid == 0);
 
   RecSink2 sink{s_recs, &s_rec_count, static_cast<uint32_t>(tid), 0u};
-  if (!(a.dbg & 1u)) lane_digit_flat(m, fv, s_info, skip_safe, c0, c1, rend, at_origin, sink);
+  lane_digit_flat(m, fv, s_info, skip_safe, c0, c1, rend, at_origin, sink);
   if (m.over) raise_err(a.err, kErrSerialLimit);
   // a lane may emit more than 65 535 matches (no synchronising byte for a long stretch); the 16-bit rank in a
   // buffered record is only read when the whole tile emitted <= the record capacity, so that is not an error
@@ -176,12 +176,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_digit_flat(ScanArgs a) {
   const uint32_t excl = block_exclusive_scan(sink.n, s_wsum, total);
   s_cnt[tid] = excl;
   const uint64_t t4 = a.prof ? clock64() : 0;
-  if (a.dbg & 2u) {
-    if (tid == 0) { s_base = atomicAdd(reinterpret_cast<unsigned long long*>(a.total), static_cast<unsigned long long>(total)); }
-    __syncthreads();
-  } else {
-    tile_lookback(a.status, a.total, a.err, tile, a.ntiles, total, &s_base);
-  }
+  tile_lookback(a.status, a.total, a.err, tile, a.ntiles, total, &s_base);
   const uint64_t t5 = a.prof ? clock64() : 0;
   if (a.prof && (tid & 63) == 0) {   // per wave: phase cycles (stage tables, stage tile, walk, scan, look-back)
     atomicAdd(reinterpret_cast<unsigned long long*>(a.prof + 0), static_cast<unsigned long long>(t1 - t0));

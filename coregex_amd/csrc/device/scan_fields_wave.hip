@@ -495,8 +495,7 @@ __global__ __launch_bounds__(kThreads, CXG_FIELDS_WAVES) void k_scan_fields_wave
   // Count (no rows wanted, no limit): nobody needs this group's place in the output, only the grand total — the look-back, in
   // which a workgroup spends more time than scanning, is replaced by a plain store and a one-workgroup sum behind the kernel
   if (a.count_sum) { if (tid == 0) a.status[group] = total; return; }
-  if (a.dbg & 2u) { if (tid == 0) s_base = 0; __syncthreads(); }     // CXG_DEBUG=2 (timing experiments, rows land in the wrong places): no look-back
-  else tile_lookback(a.status, a.total, a.err, group, a.ngroups, total, &s_base, a.epoch, a.limit, a.stop);
+  tile_lookback(a.status, a.total, a.err, group, a.ngroups, total, &s_base, a.epoch, a.limit, a.stop);
   if (a.prof && tid == 0) {
     const uint64_t pt3 = __builtin_readcyclecounter();
     atomicAdd(reinterpret_cast<unsigned long long*>(a.prof + 1), static_cast<unsigned long long>(pt1 - pt0));   // tile loop

@@ -222,7 +222,7 @@ __device__ __forceinline__ void fsm_resolve_exits(const FsmView& v, uint32_t* s_
   uint32_t entry = 0u, gx;
   if (open) {
     if (group == 0) { if (lane == 0) raise_err(a.err, 8u | (1u << 8)); return; }      // cannot happen: the input's first state is known
-    entry = (a.dbg & 8u) ? 0u : fsm_group_entry(v, a, group, s_mapu[0], cur0, cur, nlive == NT, lane);   // (CXG_DEBUG=8: timing experiment, wrong rows)
+    entry = fsm_group_entry(v, a, group, s_mapu[0], cur0, cur, nlive == NT, lane);
     const unsigned long long hit = __ballot(lane < kFsmMembers && cur0 == entry);
     gx = hit ? static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(cur), __builtin_ctzll(hit))) : 0xFFFFu;
   } else gx = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(cur), 0));
@@ -318,7 +318,6 @@ __global__ __launch_bounds__(kThreads, ((IMG > 10240 || MODE == 3 || (MODE == 2 
       if (S.ndefer == 0u) break;                       // uniform
       if (wave == 0) fsm_resolve_exits<kWavesPerBlock * tpw>(v, S.exit, S.mapx, S.mapu, a, group, lane);
       __syncthreads();
-      if (a.dbg & 4u) break;                           // (CXG_DEBUG=4: timing experiment — no second pass, rows missing)
       if (jd < tpw) issue_loads(jd);
     }
     const int j = it < tpw ? it : it - tpw;

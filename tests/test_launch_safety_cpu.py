@@ -47,3 +47,17 @@ def test_no_source_writes_through_the_scalar_data_cache():
     scalar_write = re.compile(rb"\bs_(?:buffer_|scratch_)?(?:store|atomic)_\w+|\bs_dcache_(?:wb|discard)\w*")
     assert len(names) > 100
     assert [(n, m.group().decode()) for n in names for m in [scalar_write.search(_read(n))] if m] == []
+
+
+# ---- no setting of the library leaves out part of a scan
+
+@pytest.mark.parametrize("lib", ["libcoregex_hip.so", "libcoregex_hip_rocm.so"])
+def test_no_setting_of_the_library_skips_work(lib):
+    path = os.path.join("coregex_amd", lib)
+    if not os.path.exists(os.path.join(ROOT, path)):
+        pytest.skip(f"{lib} is not built")
+    assert b"CXG_DEBUG" not in _read(path)                           # (it skipped the lane walk or the look-back and returned wrong rows)
+
+
+def test_the_benchmark_checks_its_rows_whatever_the_environment_says():
+    assert b"CXG_DEBUG" not in _read("bench.py")
