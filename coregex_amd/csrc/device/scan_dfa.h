@@ -111,7 +111,7 @@ struct ScanArgs {
   uint8_t chain[224];   // scan_chain_wave.hip: copy of the program's ChainAux (walk.hpp) — kernel arguments are read with
                         // scalar loads before the first instruction needs them, the blob would cost two dependent global loads per workgroup
   uint32_t epoch;          // wave kernels: launch epoch 1..1023 tagging the status words (0: array was zeroed, legacy)
-  uint32_t static_groups;  // wave kernels: group = blockIdx.x instead of an atomic ticket (block_common.hpp claim_group)
+  uint32_t static_groups;  // wave kernels: group = blockIdx.x instead of an atomic ticket (block_common.hpp claim_group); pair kernel: its first two groups
   uint8_t caps[40];     // scan_chain_wave.hip CAP instantiations: the program's ChainCaps (walk.hpp); caps[0] == 0: spans only
   uint32_t tiles_per_wave;  // scan_chain_wave.hip: kTilesPerWave, or kDenseTilesPerWave after a row-buffer overflow
   uint32_t max_len;     // != 0: a match longer than this raises error bit 64 (UseBoth programs, walk.hpp kFlagBothRestart)
